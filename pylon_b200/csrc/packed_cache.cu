@@ -9,6 +9,13 @@
 // step as a bfloat16, whose lowest four mantissa bits are zero and hold `zero` instead: 4 + 16 / G bits an element.  A group with an element that is
 // not finite, or a range that is not, has the word 0x7FC0: its step is NaN, and so are its values.  Steps below 2^-100 count as none (value 0).
 // Quotients, not products with 1 / step: bfloat16 inputs hit halves exactly and often, and a product would round them either way.
+//
+// All of it, and the norm and the rotation in front of it, is 32-bit arithmetic in which every operation is rounded by itself (no contracted multiply-adds) and the
+// order of the one sum, the norm's, is fixed: codes are whole numbers, and next to a border between two of them the last bit of a key decides.  So the pages are what the
+// same formulas in elementary 32-bit operations give, bit for bit; of the formulas in 64 bits they miss one code in some ten
+// million, by one, and more rarely the last bit of a group's step.  The sum of a row's d squares:
+// over 64 channels the upper half of what is left is added to the lower until one is left; over others each four channels in their order first, then the
+// halves of those.  (The orders of torch's mean over 64 and over 128 channels on this device, so that a statement in torch operations meets the same bits.)
 #include "common.cuh"
 
 namespace pylon {
@@ -95,9 +102,7 @@ __device__ __forceinline__ int page_of(const int* block_table, int table_width, 
 // ---------------------------------------------------------------------------------------------------------------------------------------------------
 // One (token, head) row to LANES lanes of a warp, eight channels to a lane: a 16-byte load of bfloat16, a 32-bit store of eight codes, and every
 // reduction (norm, a group's range) a few shuffles.  (Not const __restrict__ for what the kernel ahead writes: reads through the non-coherent path may be
-// moved ahead of the wait for it.)  Keys that are packed are normed and rotated in 64 bits: a code is a whole number, and what 32 bits round away moves one in
-// a million of them by a step; the other rows, three quarters of the work, are not.  Bound by instructions for prompt portions (2,048 tokens of 32 / 8 heads of
-// 128: 22 us, issue slots 56 % busy; its 44 MB would take 7) and by its chain of dependent loads (row, slot, page) for single tokens (3 us).
+// moved ahead of the wait for it.)
 template <typename T, typename Q, bool PACKED, int LANES>
 __global__ void __launch_bounds__(128, 6) slot_write_kernel(
     const T* qkv, int parts, long long part_stride, Q* q_out, const float* __restrict__ q_weight, const float* __restrict__ k_weight, float eps,
@@ -138,7 +143,6 @@ __global__ void __launch_bounds__(128, 6) slot_write_kernel(
     const bool there = number < heads, mine = there && c0 < d;   // lanes without a row still take part in the shuffles
     const bool is_q = head < nq, is_v = head >= nq + nkv, is_k = !is_q && !is_v;
     const bool keeps = __any_sync(0xffffffffu, there && !is_q), turns = rotary_dim > 0 && __any_sync(0xffffffffu, !is_v);
-    const bool exact = PACKED && __any_sync(0xffffffffu, is_k && there);   // (of rows that share a warp all go the longer way)
     const float* weight = is_v ? nullptr : (is_q ? q_weight : k_weight);
     float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
     if (mine && weight) load8<float>(weight + c0, w);
@@ -151,43 +155,46 @@ __global__ void __launch_bounds__(128, 6) slot_write_kernel(
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] += y[i];
     }
-    float dropped[8];   // keys that are packed: what x leaves of 64 bits
-    if (exact) {
-      double sum = 0.0;
+    if ((q_weight || k_weight) && __any_sync(0xffffffffu, weight != nullptr)) {
+      float square[8], sum;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += (double)x[i] * (double)x[i];
+      for (int i = 0; i < 8; ++i) square[i] = __fmul_rn(x[i], x[i]);
+      if constexpr (LANES == 8) {   // 64 channels: halves
 #pragma unroll
-      for (int offset = LANES / 2; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-      const double mean = sum * (1.0 / (double)d) + (double)eps, rough = (double)rsqrtf((float)mean);
-      const double inverse = weight ? rough * (1.5 - 0.5 * mean * rough * rough) : 1.0;   // one Newton step: 22 bits become 44
+        for (int offset = LANES / 2; offset > 0; offset >>= 1)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        double z = (double)x[i] * inverse * (double)w[i];
-        const double other = __shfl_sync(0xffffffffu, z, from);
-        if (!is_v) z = z * (double)c[i] + other * (double)s[i];
-        x[i] = (float)z;
-        dropped[i] = is_k ? (float)(z - (double)x[i]) : 0.f;
-      }
-    } else {
-      if (q_weight || k_weight) {
-        float sum = 0.f;
+          for (int i = 0; i < 8; ++i) square[i] = __fadd_rn(square[i], __shfl_xor_sync(0xffffffffu, square[i], offset));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+        for (int half = 4; half > 0; half >>= 1)
 #pragma unroll
-        for (int offset = LANES / 2; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-        if (weight) {
-          const float inverse = rsqrtf(sum * inverse_d + eps);
+          for (int i = 0; i < half; ++i) square[i] = __fadd_rn(square[i], square[i + half]);
+        sum = square[0];
+      } else {   // fours, then halves of those: a lane has two
+        float low = square[0], high = square[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = x[i] * inverse * w[i];
+        for (int i = 1; i < 4; ++i) {
+          low = __fadd_rn(low, square[i]);
+          high = __fadd_rn(high, square[4 + i]);
         }
-      }
-      if (turns) {
-        float other[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], from);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = is_v || !rotates ? x[i] : x[i] * c[i] + other[i] * s[i];
+        for (int offset = LANES / 2; offset > 0; offset >>= 1) {
+          low = __fadd_rn(low, __shfl_xor_sync(0xffffffffu, low, offset));
+          high = __fadd_rn(high, __shfl_xor_sync(0xffffffffu, high, offset));
+        }
+        sum = __fadd_rn(low, high);
       }
+      if (weight) {
+        const float inverse = rsqrtf(__fadd_rn(__fmul_rn(sum, inverse_d), eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inverse), w[i]);
+      }
+    }
+    if (turns) {
+      float other[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], from);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = is_v || !rotates ? x[i] : __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(other[i], s[i]));
     }
     if (mine && is_q) store8(q_out + ((size_t)t * nq + head) * d + c0, x);
     if (!keeps) continue;
@@ -224,9 +231,7 @@ __global__ void __launch_bounds__(128, 6) slot_write_kernel(
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float quotient = __fdiv_rn(x[i], step);
-          // To the nearest whole number, ties to even, by adding what leaves no bits behind the point; next to a border in 64 bits.
-          float code = (quotient + 12582912.f) - 12582912.f;
-          if (fabsf(quotient - code) > 0.4999f) code = (float)rint(((double)x[i] + (is_k ? (double)dropped[i] : 0.0)) / (double)step);
+          float code = (quotient + 12582912.f) - 12582912.f;   // to the nearest whole number, ties to even, by adding what leaves no bits behind the point
           code = fminf(fmaxf(code + zero, 0.f), 15.f) + 8388608.f;   // (NaN, of a bad group, becomes 0)
           codes |= (__float_as_uint(code) & 15u) << (4 * i);
         }
