@@ -97,13 +97,15 @@ class StepGraphs:
         """Logits wanted nowhere or at the last token of an entry: what a scheduler's ticks ask for."""
         return all(len(entry.want) == 0 or tuple(entry.want) == (len(entry.tokens) - 1,) for entry in entries)
 
-    def run(self, entries: Sequence[StepEntry]) -> Optional[torch.Tensor]:
-        """Runs a prepared step from a graph; ``None`` if it has none (the caller then runs eagerly)."""
+    def run(self, entries: Sequence[StepEntry]) -> tuple[bool, Optional[torch.Tensor]]:
+        """Runs a prepared step from a graph.  Returns whether it had one - if not, nothing was run and the caller runs eagerly - and the logits, ``None``
+        where none are wanted: a step must not run twice, its state would be advanced and its weights added to the masses twice."""
         if self.decode_only(entries):
-            return self.run_decode(entries)
+            logits = self.run_decode(entries)
+            return logits is not None, logits   # (every row of such a step wants logits)
         if self.pad_steps and self.scheduler_shaped(entries):
             return self.run_padded(entries)
-        return None
+        return False, None
 
     def replays_whole(self, entries: Sequence[StepEntry]) -> bool:
         """Whether ``run`` will replay this step from a graph it has already: the model's kernels are then queued by one
@@ -203,10 +205,10 @@ class StepGraphs:
         key = (bucket_rows(len(ones)), bucket_rows(len(portions)), bucket_tokens(sum(len(entry.tokens) for entry in portions)))
         return key, ones, portions
 
-    def run_padded(self, entries: Sequence[StepEntry]) -> Optional[torch.Tensor]:
+    def run_padded(self, entries: Sequence[StepEntry]) -> tuple[bool, Optional[torch.Tensor]]:
         key, ones, portions = self.padded_size(entries)
         if key in self.failed:
-            return None
+            return False, None
         one_rows, portion_rows, portion_tokens = key
         wanted = sum(1 for entry in entries if entry.want)
         captured = self.captured_padded.get(key)
@@ -216,7 +218,7 @@ class StepGraphs:
             # of decoding requests) is not worth one; a size that comes back is.
             self.seen_padded[key] = self.seen_padded.get(key, 0) + 1
             if len(self.captured_padded) >= MAX_PADDED_GRAPHS or (self.seen_padded[key] < 2 and not self.capture_at_once):
-                return None
+                return False, None
             # every row may want logits at its last token
             layout = StepLayout(tokens=one_rows + portion_tokens, rows=one_rows + portion_rows, logits=one_rows + portion_rows, table_widths=self.widths(portion_tokens),
                                 evicts=self.cache.evicts)
@@ -231,12 +233,12 @@ class StepGraphs:
             step.row_tokens = (1,) * one_rows + (portion_tokens,) * portion_rows
             captured = self._capture(key, step, self.cache.layer_caches(tables), layout, static_buffer, entries)
             if captured is None:
-                return None
+                return False, None
             self.captured_padded[key] = captured
         host = torch.empty(captured.layout.total, dtype=torch.int32, pin_memory=True)
         function.fill_padded(ones, portions, entries, captured.layout, host.numpy(), one_rows)
         logits = self._replay(captured, host, "padded", self.step_function.sampled_source(entries))
-        return logits[:wanted] if wanted else None
+        return True, logits[:wanted] if wanted else None
 
 
 DecodeGraphs = StepGraphs   # the name this class had while it replayed decode steps only

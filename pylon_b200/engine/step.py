@@ -295,10 +295,10 @@ class StepFunction:
             # launch or not at all (the copy would cost a decode step as much as reading the states does)
             if self.graphs is None or not self.graphs.replays_whole(entries):
                 saved_state = self.cache.save_state([request for request, _ in batch])
-            logits = None
+            ran, logits = False, None
             if self.graphs is not None:
-                logits = self.graphs.run(entries)
-            if logits is None:
+                ran, logits = self.graphs.run(entries)
+            if not ran:
                 if saved_state is None:
                     saved_state = self.cache.save_state([request for request, _ in batch])
                 logits = self._run_eager(entries)
