@@ -1794,8 +1794,9 @@ __global__ void combine_splits_kernel(const float* __restrict__ partial_out, con
   allow_dependents();   // only now: a kernel that is itself still waiting must not pull the next one onto the SMs
   const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (item >= items) return;
+  const int token = (int)(item / nq);
+  if (token < q_start[0] || token >= q_start[num_rows]) return;   // a token of none of these rows: nobody has left parts of it
   if (skip_small) {
-    const int token = (int)(item / nq);
     int lo = 0, hi = num_rows - 1;   // the last row that starts at or before the token
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;

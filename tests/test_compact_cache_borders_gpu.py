@@ -72,3 +72,32 @@ def test_portions_are_packed_bit_for_bit(dtype, nq, nkv, d, group, page):
             codes, words = packed_32(values, group)
             assert torch.equal(pages.words[page_of, :, at], words) and torch.equal(pages.codes[page_of, :, at], codes)
     ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+# ---------------------------------------------------------------------------------------
+# attention over unpacked contexts
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("nq, nkv, d, counts, lengths", [
+    (4, 2, 96, [64, 1, 9, 40], [700, 650, 9, 300]), (2, 2, 256, [1, 30, 30, 30], [600, 30, 500, 77]), (8, 1, 32, [20], [900]), (4, 2, 64, [64, 1, 9, 40], [700, 650, 9, 300]),
+])
+def test_rows_that_are_unpacked_a_few_at_a_time(nq, nkv, d, counts, lengths, known, monkeypatch):
+    """Every batch of rows leaves the others' results, and padding tokens' rows, as they are, also where few query tiles over long contexts are cut into parts."""
+    from pylon_b200.kernels import ops
+
+    page, bound, tokens = 16, 2000, sum(counts)
+    table, pool, q_start, kv_len, row, slots = tables(counts, lengths, page)
+    k_pages, v_pages = random_pages(pool, nkv, page, d, 32), random_pages(pool, nkv, page, d, 32)
+    q = torch.randn(tokens + 3, nq * d, device=DEVICE).bfloat16()
+    row, slots = torch.cat((row, ints([-1] * 3))), torch.cat((slots, ints([0] * 3)))
+    expected, size = plain.attention(q[:tokens], k_pages, v_pages, counts, lengths, table, nq, d ** -0.5)
+    for rows_at_once in (len(counts), 3, 1):
+        monkeypatch.setattr(ops, "UNPACKED_BYTES", rows_at_once * 32 * 64 * nkv * d * 4)
+        out = torch.full((tokens + 3, nq * d), 3.0, device=DEVICE).bfloat16()
+        for before in (None, float("nan")):      # what fresh memory held before reaches nobody
+            torch.full((1 << 24,), 0.0 if before is None else before, device=DEVICE)
+            ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, table, nq, max(counts), bound, out=out, row_tokens=tuple(counts) if known else None)
+            assert (out[tokens:] == 3.0).all()
+            # weights of 8 bits and the result's rounding; scores in 32 bits
+            assert ((out[:tokens].double() - expected).abs() <= HALF[torch.bfloat16] * (expected.abs() + size) + 2.0 ** -14 * size).all()
+    ops.raise_on_kernel_errors(torch.device(DEVICE))
