@@ -114,6 +114,7 @@ __device__ __forceinline__ float word_zero(unsigned word) { return (float)(int)(
 // A row's stretch of tiles.
 struct RowPlan {
   int first_token, tokens, length, first_tile, tiles;
+  int oldest;   // the first slot that a token sees; the pages of those before it may be gone
 };
 __device__ __forceinline__ RowPlan row_plan(const PackedParams& p, int row) {
   RowPlan r;
@@ -124,10 +125,10 @@ __device__ __forceinline__ RowPlan row_plan(const PackedParams& p, int row) {
     r.tokens = p.last;
   }
   r.length = min(p.kv_len[row], p.most_slots);
-  r.first_tile = 0;
-  r.tiles = 0;
+  r.first_tile = r.tiles = r.oldest = 0;
   if (r.tokens > 0 && r.tokens <= p.most_packed / p.group && r.length > 0) {
-    if (p.window > 0) r.first_tile = max(0, r.length - r.tokens - p.window + 1) / TILE;
+    if (p.window > 0) r.oldest = max(0, r.length - r.tokens - p.window + 1);
+    r.first_tile = r.oldest / TILE;
     r.tiles = (r.length + TILE - 1) / TILE - r.first_tile;
   }
   return r;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void copy_stage(const PackedParams& p, const Cursor& 
       ++logical;
     }
     int page = 0;
-    if (valid > 0) {
+    if (valid > 0 && key0 + 16 * half + valid > c.plan.oldest) {
       page = table[logical];
       if (page < 0 || page >= p.num_pages) {
         if (left == 0) atomicExch(p.error, PYLON_ERROR_BAD_PAGE);
@@ -275,7 +276,7 @@ __device__ __forceinline__ void copy_stage(const PackedParams& p, const Cursor& 
   } else {   // any page size: a page for every key, and the words by hand
     const int own = key0 + lane;
     size_t own_row = 0;
-    bool there = own < c.plan.length;
+    bool there = own < c.plan.length && own >= c.plan.oldest;
     if (there) {
       const int page = table[own / p.page_size];
       if (page < 0 || page >= p.num_pages) {

@@ -279,8 +279,9 @@ __global__ void __launch_bounds__(256) read_packed_kernel(const unsigned* k_page
   }
 }
 
-// Rows' contexts as plain pages of `out_page` slots: row r's slot j goes to page r * out_width + j / out_page.  Slots from a row's length to the next
-// multiple of 128 become zeros, so that a kernel that reads whole tiles meets no old numbers.  A kernel that multiplies masked weights of zero into whole
+// Rows' contexts as plain pages of `out_page` slots: row r's slot j goes to page r * out_width + j / out_page.  With a window only from the first slot that one of the
+// row's tokens sees: the pages before it may be gone.  Slots from the multiple of 128 below that one, and from a row's length to the next
+// multiple of 128, become zeros, so that a kernel that reads whole tiles meets no old numbers.  A kernel that multiplies masked weights of zero into whole
 // tiles of values would hand a value that is not a number to tokens that do not see it; so a slot with such a value gets a key that is not one (masked
 // scores are chosen away, not multiplied) and zeros in its place: who sees the slot has no number in any channel, nobody else is touched.  Bound by
 // instructions (issue slots 77 % busy): contexts of 4,501 and some 3,000 slots of 8 heads of 128 in 14 us, 2.7 TB/s.
@@ -298,7 +299,7 @@ __device__ __forceinline__ uint4 unpack8(unsigned codes, unsigned word) {   // e
 }
 template <typename Q>
 __global__ void __launch_bounds__(256) unpack_pages_kernel(const unsigned* k_pages, const unsigned short* k_words, const unsigned* v_pages, const unsigned short* v_words, Q* k_out,
-                                                           Q* v_out, const int* kv_len, const int* block_table, int table_width, int page_size, int num_pages, int nkv, int d,
+                                                           Q* v_out, const int* q_start, const int* kv_len, int window, const int* block_table, int table_width, int page_size, int num_pages, int nkv, int d,
                                                            int group, int out_page, int out_width, int* lengths, int* error) {
   grid_dependency_wait();
   allow_dependents();
@@ -309,10 +310,11 @@ __global__ void __launch_bounds__(256) unpack_pages_kernel(const unsigned* k_pag
   }
   if ((int)threadIdx.x >= at_once * chunks) return;
   const int length = min(kv_len[row], out_width * out_page), end = min((length + 127) & ~127, out_width * out_page);
-  for (int slot = blockIdx.x * at_once + threadIdx.x / chunks; slot < end; slot += gridDim.x * at_once) {
+  const int oldest = window > 0 ? max(0, length - (q_start[row + 1] - q_start[row]) - window + 1) : 0;
+  for (int slot = (oldest & ~127) + blockIdx.x * at_once + threadIdx.x / chunks; slot < end; slot += gridDim.x * at_once) {
     uint4 k = make_uint4(0u, 0u, 0u, 0u), v = make_uint4(0u, 0u, 0u, 0u);
     float k32[8] = {}, v32[8] = {};
-    if (slot < length) {
+    if (slot >= oldest && slot < length) {
       const int page = page_of(block_table, table_width, num_pages, row, slot, page_size);
       if (page >= 0) {
         const size_t src = ((size_t)page * nkv + head) * page_size + slot % page_size;
@@ -421,19 +423,19 @@ extern "C" int pylon_read_packed(const void* k_pages, const void* k_words, const
   PYLON_CHECK_LAUNCH("read_packed");
 }
 
-extern "C" int pylon_unpack_pages(const void* k_pages, const void* k_words, const void* v_pages, const void* v_words, void* k_out, void* v_out, const int* kv_len, const int* block_table,
-                                  int table_width, int page_size, int num_pages, int nkv, int d, int group, int rows, int max_kv, int out_page, int out_width, int* lengths,
+extern "C" int pylon_unpack_pages(const void* k_pages, const void* k_words, const void* v_pages, const void* v_words, void* k_out, void* v_out, const int* q_start, const int* kv_len, int window,
+                                  const int* block_table, int table_width, int page_size, int num_pages, int nkv, int d, int group, int rows, int max_kv, int out_page, int out_width, int* lengths,
                                   int out_dtype, int* error, cudaStream_t stream) {
   if (rows == 0) return 0;
   if (int code = check_sizes("unpack_pages", nkv, d, group, page_size, table_width, num_pages)) return code;
   if (!lengths || !error) PYLON_REFUSE("unpack_pages: room for the lengths and an error word are needed");
-  if (out_page < 1 || out_width < 1 || max_kv < 1 || nkv > 65535 || rows > 65535) PYLON_REFUSE("unpack_pages: %d rows, %d KV heads, pages of %d, %d a row", rows, nkv, out_page, out_width);
+  if (window < 0 || out_page < 1 || out_width < 1 || max_kv < 1 || nkv > 65535 || rows > 65535) PYLON_REFUSE("unpack_pages: %d rows, %d KV heads, pages of %d, %d a row", rows, nkv, out_page, out_width);
   const int at_once = 256 / (d / 8);
   const long long wanted = ((long long)max_kv + 127 + at_once - 1) / at_once, most = 1 + 16ll * multiprocessors() / ((long long)rows * nkv);
 #define PYLON_UNPACK(Q)                                                                                                                                                     \
   launch_dependent(unpack_pages_kernel<Q>, dim3((unsigned)(wanted < most ? wanted : most), nkv, rows), dim3(256), 0, stream, (const unsigned*)k_pages,                         \
-                   (const unsigned short*)k_words, (const unsigned*)v_pages, (const unsigned short*)v_words, (Q*)k_out, (Q*)v_out, kv_len, block_table, table_width, page_size, \
-                   num_pages, nkv, d, group, out_page, out_width, lengths, error)
+                   (const unsigned short*)k_words, (const unsigned*)v_pages, (const unsigned short*)v_words, (Q*)k_out, (Q*)v_out, q_start, kv_len, window, block_table, table_width, \
+                   page_size, num_pages, nkv, d, group, out_page, out_width, lengths, error)
   if (out_dtype == PYLON_DTYPE_F32) PYLON_UNPACK(float);
   else if (out_dtype == PYLON_DTYPE_BF16) PYLON_UNPACK(__nv_bfloat16);
   else PYLON_REFUSE("unpack_pages: unknown dtype %d", out_dtype);

@@ -337,8 +337,8 @@ _SIGNATURES = {
                              c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
         "pylon_read_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                               c_void_p, c_void_p],
-        "pylon_unpack_pages": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                               c_int, c_void_p, c_int, c_void_p, c_void_p],
+        "pylon_unpack_pages": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                               c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     },
     "attention_packed.cu": {
         "pylon_attention_packed_blocks": [c_int, c_int, c_int, c_int],
@@ -2436,6 +2436,7 @@ def paged_attention_packed(
     ``slots`` (int32 ``[T]``): each token's slot in its row (its position, where nothing was evicted); a token sees the slots up to its own, with ``window``
     the last ``window`` of them.  ``kv_len`` counts slots: a row's first new token has slot ``kv_len - (q_start[r + 1] - q_start[r])``.  The other arguments are
     :func:`paged_attention`'s; ``q`` is bfloat16 or float32, the result ``[T, nq * d]`` in its dtype.  Padding tokens' rows of the result are not written.
+    Pages that a window has passed may be gone (-1 in the table).
 
     Head sizes: multiples of 32 up to 256.  bfloat16 queries of rows of at most 16 packed query rows (tokens x query heads of a KV head) run on a tensor-core kernel
     over the codes where the head size is 64 or 128 (``csrc/attention_packed.cu``; scores and sums are 32-bit, a weight times the step of its values is rounded to
@@ -2547,8 +2548,8 @@ def _attention_unpacked(q: torch.Tensor, k_pages: PackedPages, v_pages: PackedPa
     for begin in range(first, after, at_once):
         end = min(after, begin + at_once)
         _check(library, library.pylon_unpack_pages(
-            _ptr(k_pages.codes), _ptr(k_pages.words), _ptr(v_pages.codes), _ptr(v_pages.words), _ptr(k), _ptr(v), kv_len.data_ptr() + 4 * begin, block_table.data_ptr() + 4 * begin * width,
-            width, page_size, pages, nkv, d, group, end - begin, int(max_kv), 64, out_width, _ptr(lengths), _dtype_code(q.dtype), _error_address(device.index, 1), _stream()))
+            _ptr(k_pages.codes), _ptr(k_pages.words), _ptr(v_pages.codes), _ptr(v_pages.words), _ptr(k), _ptr(v), q_start.data_ptr() + 4 * begin, kv_len.data_ptr() + 4 * begin, int(window or 0),
+            block_table.data_ptr() + 4 * begin * width, width, page_size, pages, nkv, d, group, end - begin, int(max_kv), 64, out_width, _ptr(lengths), _dtype_code(q.dtype), _error_address(device.index, 1), _stream()))
         if shared:
             split_library = _library("attention_tcgen05.cu", {**_SPLIT_KEYS, "PYLON_HEAD_DIM": d})
             _check(split_library, split_library.pylon_paged_attention_tcgen05_parts(

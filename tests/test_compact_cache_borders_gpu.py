@@ -101,3 +101,35 @@ def test_rows_that_are_unpacked_a_few_at_a_time(nq, nkv, d, counts, lengths, kno
             # weights of 8 bits and the result's rounding; scores in 32 bits
             assert ((out[:tokens].double() - expected).abs() <= HALF[torch.bfloat16] * (expected.abs() + size) + 2.0 ** -14 * size).all()
     ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq, nkv, d, page, counts, lengths, window", [
+    (8, 2, 128, 16, [1, 2, 1], [700, 301, 40], 100), (8, 2, 128, 24, [1, 1], [700, 301], 33), (8, 2, 64, 256, [1, 1], [900, 1025], 1), (8, 2, 128, 64, [40, 1], [800, 500], 90),
+    (4, 2, 64, 7, [70], [500], 128), (8, 2, 96, 16, [1, 30], [700, 900], 65), (32, 8, 128, 64, [200], [4600], 300),
+])
+def test_pages_that_a_window_has_passed_are_gone(dtype, nq, nkv, d, page, counts, lengths, window):
+    """A cache gives back the pages that no token sees any more; the table holds -1 in their places, which is no error and no page."""
+    from pylon_b200.kernels import ops
+
+    table, pool, q_start, kv_len, row, slots = tables(counts, lengths, page)
+    k_pages, v_pages = random_pages(pool, nkv, page, d, 32), random_pages(pool, nkv, page, d, 32)
+    q = torch.randn(sum(counts), nq * d, device=DEVICE).to(dtype)
+    gone = table.clone()
+    for r, (count, length) in enumerate(zip(counts, lengths)):
+        first = max(0, length - count - window + 1) // page
+        assert first > 0 or length < window + count
+        gone[r, :first] = -1
+    expected, size = plain.attention(q, k_pages, v_pages, counts, lengths, table, nq, d ** -0.5, window)
+    for row_tokens in (None, tuple(counts)):
+        results = [ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, each, nq, max(counts), max(lengths), window=window, row_tokens=row_tokens)
+                   for each in (table, gone)]
+        ops.raise_on_kernel_errors(torch.device(DEVICE))
+        assert torch.equal(*results)
+        assert ((results[1].double() - expected).abs() <= HALF[dtype] * (expected.abs() + size) + 2.0 ** -14 * size).all()
+    # a page that a token sees is still missed
+    last = max(0, lengths[0] - counts[0] - window + 1) // page
+    gone[0, last] = -1
+    ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, gone, nq, max(counts), max(lengths), window=window, row_tokens=tuple(counts))
+    with pytest.raises(ops.KernelError, match="attention"):
+        ops.raise_on_kernel_errors(torch.device(DEVICE))
