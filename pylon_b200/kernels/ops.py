@@ -2469,7 +2469,8 @@ def paged_attention_packed(
         raise KernelError(f"{what}: out has the wrong shape or dtype")
     device = _on_current_device(what, q, slots, token_row, q_start, kv_len, block_table, out, *k_pages, *v_pages)
     if out is not None and out.data_ptr() % 16:
-        return out.copy_(paged_attention_packed(q, k_pages, v_pages, slots, token_row, q_start, kv_len, block_table, nq, max_q, max_kv, window, scale, None, row_tokens))
+        aligned = out.clone()   # padding tokens' rows with what they hold
+        return out.copy_(paged_attention_packed(q, k_pages, v_pages, slots, token_row, q_start, kv_len, block_table, nq, max_q, max_kv, window, scale, aligned, row_tokens))
     if out is None:
         out = torch.empty((tokens, nq * d), dtype=q.dtype, device=q.device)
     if tokens == 0 or rows == 0:

@@ -133,3 +133,22 @@ def test_pages_that_a_window_has_passed_are_gone(dtype, nq, nkv, d, page, counts
     ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, gone, nq, max(counts), max(lengths), window=window, row_tokens=tuple(counts))
     with pytest.raises(ops.KernelError, match="attention"):
         ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts, lengths, d", [([1, 2], [300, 40], 64), ([40, 1], [90, 700], 128), ([40, 1], [90, 700], 96)])
+def test_padding_rows_of_a_result_anywhere_in_memory(counts, lengths, d, dtype):
+    """A result that does not start on 16 bytes is worked out elsewhere: padding tokens' rows are left alone all the same."""
+    from pylon_b200.kernels import ops
+
+    nq, nkv, page, tokens = 8, 2, 16, sum(counts)
+    table, pool, q_start, kv_len, row, slots = tables(counts, lengths, page)
+    k_pages, v_pages = random_pages(pool, nkv, page, d, 32), random_pages(pool, nkv, page, d, 32)
+    q = torch.randn(tokens + 2, nq * d, device=DEVICE).to(dtype)
+    row, slots = torch.cat((row, ints([-1, -1]))), torch.cat((slots, ints([0, 0])))
+    torch.full((1 << 24,), float("nan"), device=DEVICE)      # what fresh memory holds
+    out = torch.full(((tokens + 2) * nq * d + 1,), 3.0, dtype=dtype, device=DEVICE)[1:].view(tokens + 2, nq * d)
+    assert ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, table, nq, max(counts), max(lengths), out=out).data_ptr() == out.data_ptr()
+    wanted = ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, table, nq, max(counts), max(lengths))
+    assert (out[tokens:] == 3.0).all() and torch.equal(out[:tokens], wanted[:tokens])
+    ops.raise_on_kernel_errors(torch.device(DEVICE))
