@@ -2533,6 +2533,8 @@ def _attention_unpacked(q: torch.Tensor, k_pages: PackedPages, v_pages: PackedPa
     """Rows ``first`` to ``after`` of a step: their contexts as plain pages of 64 slots in the dtype of ``q`` (exact, see :class:`PackedPages`), side by side, and attention over those:
     where the query tiles fill the device :func:`paged_attention`, else the kernel that shares a tile's keys among blocks.  Returns whether all of the rows
     are done: without ``counts`` the latter leaves out those of at most 16 packed query rows."""
+    if counts is not None and not any(counts[first:after]):   # padding tokens alone
+        return True
     pages, nkv, page_size, d, group = _packed_sizes(k_pages, "paged_attention_packed")
     width, out_width, device = block_table.shape[1], -(-max_kv // 64), q.device
     at_once = max(1, UNPACKED_BYTES // (out_width * 64 * nkv * d * 2 * q.element_size()))

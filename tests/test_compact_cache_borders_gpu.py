@@ -152,3 +152,17 @@ def test_padding_rows_of_a_result_anywhere_in_memory(counts, lengths, d, dtype):
     wanted = ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, table, nq, max(counts), max(lengths))
     assert (out[tokens:] == 3.0).all() and torch.equal(out[:tokens], wanted[:tokens])
     ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 96), (torch.bfloat16, 128), (torch.float32, 64)])
+def test_rows_that_the_host_knows_to_be_empty(dtype, d):
+    """A padded step whose rows all are without tokens."""
+    from pylon_b200.kernels import ops
+
+    k_pages, v_pages = random_pages(3, 2, 16, d, 32), random_pages(3, 2, 16, d, 32)
+    out, nothing = torch.full((2, 4 * d), 3.0, dtype=dtype, device=DEVICE), ints([-1, -1])
+    for max_q in (1, 40):
+        for held in (0, 20):
+            ops.paged_attention_packed(torch.zeros_like(out), k_pages, v_pages, ints([0, 0]), nothing, ints([0, 0, 0]), ints([held, held]), ints([[0, 1], [2, 0]]), 4, max_q, 32, out=out, row_tokens=(0, 0))
+    assert (out == 3.0).all()
+    ops.raise_on_kernel_errors(torch.device(DEVICE))
