@@ -351,14 +351,17 @@ extern "C" int pylon_evict_slots(const float* mass, const int* places, const int
       moves.unit[moves.count++] = unit;
     }
   }
-  // A cluster of as many blocks as leave each at most 4,096 slots, up to eight; their keys in shared memory as long as they fit.
-  const int slots = table_width * page_size, longest = max_kv < slots ? max_kv : slots;
-  unsigned ranks = 1;
-  while (ranks < 8 && (longest + (int)ranks - 1) / (int)ranks > 4096) ranks *= 2;
-  const int stretch = ((longest + (int)ranks - 1) / (int)ranks + 31) & ~31, most_groups = (((slots + (int)ranks - 1) / (int)ranks + 31) & ~31) / 32;
-  const int staged = stretch <= EVICT_STAGED ? stretch : 0;
-  const size_t smem = (2 * (size_t)staged + 3 * (size_t)most_groups) * 4;
-  if (smem > EVICT_SMEM) PYLON_REFUSE("evict_slots: %d slots to a row are too many", slots);
+  // A cluster of as many blocks as leave each at most 4,096 slots and room for the numbers of all that its table could hold, up to eight; their keys in shared memory
+  // as long as they fit.
+  const long long slots = (long long)table_width * page_size, longest = max_kv < slots ? max_kv : slots;
+  long long ranks = 1, staged, smem;
+  for (;; ranks *= 2) {
+    const long long stretch = ((longest + ranks - 1) / ranks + 31) & ~31ll, most_groups = (((slots + ranks - 1) / ranks + 31) & ~31ll) / 32;
+    staged = stretch <= EVICT_STAGED ? stretch : 0;
+    smem = (2 * staged + 3 * most_groups) * 4;
+    if (ranks == 8 || ((longest + ranks - 1) / ranks <= 4096 && smem <= EVICT_SMEM)) break;
+  }
+  if (smem > EVICT_SMEM) PYLON_REFUSE("evict_slots: %lld slots to a row are too many", slots);
   static bool ready[MAX_DEVICES] = {};
   bool& set = ready[current_device_slot()];
   if (!set) {
@@ -370,8 +373,8 @@ extern "C" int pylon_evict_slots(const float* mass, const int* places, const int
   int* holes = lists;
   int* movers = lists + pairs * room;
   int* counts = lists + 2 * pairs * room;
-  launch_dependent_cluster(evict_select_kernel, dim3(ranks, nkv, rows), dim3(EVICT_THREADS), smem, stream, ranks, mass, places, kv_len, block_table, table_width, page_size, num_pages,
-                           nkv, keep, keep_first, keep_recent, holes, movers, room, counts, held, staged, error);
+  launch_dependent_cluster(evict_select_kernel, dim3((unsigned)ranks, nkv, rows), dim3(EVICT_THREADS), (size_t)smem, stream, (unsigned)ranks, mass, places, kv_len, block_table, table_width, page_size, num_pages,
+                           nkv, keep, keep_first, keep_recent, holes, movers, room, counts, held, (int)staged, error);
   const int most = max_kv > keep ? (max_kv - keep < keep ? max_kv - keep : keep) : 0;
   if (most > 0) {
     const long long wanted = (most + 8 * MOVE_SLOTS - 1) / (8 * MOVE_SLOTS), fill = 1 + 16ll * multiprocessors() / pairs;

@@ -166,3 +166,27 @@ def test_rows_that_the_host_knows_to_be_empty(dtype, d):
             ops.paged_attention_packed(torch.zeros_like(out), k_pages, v_pages, ints([0, 0]), nothing, ints([0, 0, 0]), ints([held, held]), ints([[0, 1], [2, 0]]), 4, max_q, 32, out=out, row_tokens=(0, 0))
     assert (out == 3.0).all()
     ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+# ---------------------------------------------------------------------------------------
+# eviction
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("length, width", [(300, 1_500_000 // 16), (4096, 500_000 // 16), (4000, 1_500_000 // 16), (30_000, 1_500_000 // 16)])
+def test_short_rows_of_wide_tables(length, width):
+    """Tables of up to 1.5 million slots to a row are taken, however short the rows are."""
+    from pylon_b200.kernels import ops
+
+    nkv, page, keep = 2, 16, 100
+    table, pool, _, kv_len, _, _ = tables([0], [length], page)
+    mass = torch.rand(pool, nkv, page, device=DEVICE)
+    places = torch.zeros(pool, nkv, page, dtype=torch.int32, device=DEVICE)
+    where, at = plain.row_slots(table[0], length, page)
+    for head in range(nkv):
+        places[where, head, at] = torch.randperm(length, device=DEVICE).int()
+    rows = torch.randn(pool, nkv, page, 3, device=DEVICE)
+    expected = plain.evict(mass, places, (rows,), [length], table, keep, 4, 8)
+    wide = torch.full((1, width), -1, dtype=torch.int32, device=DEVICE)
+    wide[:, : table.shape[1]] = table
+    held = ops.evict_slots(mass, places, (rows,), kv_len, wide, length, keep, keep_first=4, keep_recent=8)
+    assert held.tolist() == [keep] and all(torch.equal(got, wanted) for got, wanted in zip((mass, places, rows), expected))
+    ops.raise_on_kernel_errors(torch.device(DEVICE))
