@@ -113,7 +113,7 @@ class Engine:
     def _pool_pages(self, needs, dtype: torch.dtype, page_size: int) -> dict:
         """Pages for every cache group (by its :class:`~pylon_b200.parts.base.KVNeed`).  With ``max_cache_tokens`` the
         pool holds that many tokens; else it takes what is left of the allowed share of the device after the weights,
-        less room for the activations of one full step (raun6k/Pylon sizes its pool the same way,
+        less room for the activations of one full step and, with a compact cache, for its operators' workspace (raun6k/Pylon sizes its pool the same way,
         src/pylon/kv/budget.py:70-113).  A windowed group is given only what ``max_batch_size`` requests can hold of it
         at once, and the groups that keep everything share the rest."""
         slots, chunk, longest = self.config.max_batch_size, self.config.prefill_chunk_size, self.spec.max_positions
@@ -129,6 +129,9 @@ class Engine:
             return {}
         free, total = torch.cuda.mem_get_info(self.device)
         activation_room = chunk * self.spec.width * 64
+        if self.config.cache_bits != 16 or self.config.cache_keep is not None:
+            # (padded steps have up to twice the rows and an eighth more tokens; graphs keep a workspace of their own beside that of eager steps)
+            activation_room += self.model.workspace_bytes(2 * slots, chunk + chunk // 8 + 2 * slots, longest) * (2 if self.config.cuda_graphs else 1)
         budget = int(total * self.config.max_gpu_utilization) - (total - free) - activation_room
         windowed = {kv: pages for kv, pages in most.items() if kv.bounded}
         budget -= sum(pages * page_bytes[kv] for kv, pages in windowed.items())

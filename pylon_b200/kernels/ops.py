@@ -2718,6 +2718,32 @@ def evict_slots(
     return held
 
 
+def compact_cache_workspace(rows: int, tokens: int, longest: int, nq: int, nkv: int, d: int, element: int, packed: bool, votes: int, multiprocessors: int) -> int:
+    """The most bytes that a layer's :func:`paged_attention_packed` (``packed``) and :func:`attention_mass` (``votes`` > 0 for each row) take beside their arguments and
+    results in a step of ``tokens`` tokens in ``rows`` rows, whose ``max_kv`` is ``longest``: what an engine keeps free of pages."""
+    room = 0
+    if packed:
+        row = 2 * -(-longest // 64) * 64 * nkv * d * element
+        room = min(rows * row, max(UNPACKED_BYTES, row)) + 4096 * (rows + 1)     # unpacked contexts
+        if element == 4 or rows > 1024:                                          # or the parts of the 32-bit kernel
+            room = max(room, min(1 << 28, 4 * tokens * nq * -(-longest // 128) * (d + 2)))
+        # parts of query tiles (their tiles times the blocks to each are at most two to an SM) and of small rows beside them; parts of runs over the codes
+        room += 4 * (d + 2) * (256 * multiprocessors + 128 * rows * nkv + 128 * multiprocessors)
+    if votes:
+        columns, pairs = votes * (nq // nkv), rows * nkv
+        few = min(1 << 29, 64 * pairs * longest) + 8 * 32 * 4 * multiprocessors + 16 * pairs * 16 * (1 + -(-longest // 64))      # kept scores, and their parts
+        if element == 4:
+            many = 8 * rows * votes * nq
+        elif d in (64, 128):
+            many = 8 * columns * max(multiprocessors, pairs * -(-longest // 2048))
+        else:
+            chunks = -(-columns // 64)
+            stretch = 64 * min(8, max(1, pairs * -(-longest // 64) * chunks // (4 * multiprocessors)))
+            many = 8 * pairs * columns * (1 + -(-longest // stretch)) + pairs * chunks * 128 * d
+        room += max(few, many)
+    return room
+
+
 # ---------------------------------------------------------------------------------------
 # sampling
 # ---------------------------------------------------------------------------------------

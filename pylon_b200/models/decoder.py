@@ -115,6 +115,10 @@ class DecoderModel:
             for run in self.spec.order
         ]
 
+    def workspace_bytes(self, rows: int, tokens: int, longest: int) -> int:
+        """The most that a layer takes for a while (see :meth:`~pylon_b200.parts.base.Mixer.workspace_bytes`); layers run one after another."""
+        return max((self.blocks[run.layer].mixer.workspace_bytes(rows, tokens, longest) for run in self.spec.order), default=0)
+
     # -- run -----------------------------------------------------------------------------
     def forward(self, step: StepView, caches: Sequence[LayerCache], taps: Optional[list] = None) -> Optional[torch.Tensor]:
         """Runs the step's tokens; returns float32 logits ``[num_logits, vocab]`` at

@@ -317,6 +317,15 @@ class GroupedQueryAttention(Mixer):
             raise ValueError(f"cache_keep: heads of {self.head_dim} channels; a multiple of 16 up to 256 is needed")
         self.compact = compact
 
+    def workspace_bytes(self, rows: int, tokens: int, longest: int) -> int:
+        compact = self.compact
+        if compact is None:
+            return 0
+        if compact.keep is not None:   # what a request holds at most, a step's tokens included
+            longest = min(longest, compact.keep + compact.slack + tokens)
+        return ops.compact_cache_workspace(rows, tokens, longest, self.n_heads, self.n_kv_heads, self.head_dim, self.w_qkv.element_size(), compact.bits == 4,
+                                           0 if compact.keep is None else compact.votes, ops._multiprocessors(self.w_qkv.device))
+
     # -- run -----------------------------------------------------------------------------
     def forward(self, h: torch.Tensor, step: StepView, cache: LayerCache) -> torch.Tensor:
         if self.stacked:

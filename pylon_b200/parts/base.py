@@ -298,6 +298,10 @@ class Mixer(Part):
         """Asks for a compact cache from now on (before the weights are loaded); a mixer that cannot keep one says so."""
         raise ValueError(f"{type(self).__name__} keeps no compact cache: cache_bits and cache_keep are for models whose layers are grouped-query attention with rotated heads")
 
+    def workspace_bytes(self, rows: int, tokens: int, longest: int) -> int:
+        """What a step of ``tokens`` tokens in ``rows`` rows of up to ``longest`` slots takes for a while beyond what every step's activations take."""
+        return 0
+
     def forward(self, h: torch.Tensor, step: StepView, cache: LayerCache) -> torch.Tensor:
         """Returns the delta for the residual stream (see :class:`ResidualStream`)."""
         raise NotImplementedError

@@ -190,3 +190,42 @@ def test_short_rows_of_wide_tables(length, width):
     held = ops.evict_slots(mass, places, (rows,), kv_len, wide, length, keep, keep_first=4, keep_recent=8)
     assert held.tolist() == [keep] and all(torch.equal(got, wanted) for got, wanted in zip((mass, places, rows), expected))
     ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+# ---------------------------------------------------------------------------------------
+# workspaces
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nq, nkv, d, counts, longest, known", [
+    (32, 8, 128, [1] * 16, 40_000, True), (32, 8, 128, [1] * 3 + [500], 40_000, True), (32, 8, 128, [1] * 3 + [500], 40_000, False), (8, 2, 96, [1] * 5 + [100, 20], 9_000, True),
+    (16, 2, 64, [1] * 40 + [30], 70_000, False), (8, 8, 256, [4, 4], 2_000, True), (4, 2, 64, [1], 300_000, True),
+])
+def test_what_is_taken_for_a_while(dtype, nq, nkv, d, counts, longest, known):
+    """An engine leaves this much free for the operators of a compact cache: calls that are planned for the longest contexts take no more."""
+    from pylon_b200.kernels import ops
+
+    page, rows, tokens, votes = 256, len(counts), sum(counts), 64
+    lengths = [count + 20 for count in counts]
+    table, pool, q_start, kv_len, row, slots = tables(counts, lengths, page)
+    wide = torch.zeros(rows, -(-longest // page), dtype=torch.int32, device=DEVICE)
+    wide[:, : table.shape[1]] = table
+    k_pages, v_pages = random_pages(pool, nkv, page, d, 32), random_pages(pool, nkv, page, d, 32)
+    q, out = torch.randn(tokens, nq * d, device=DEVICE).to(dtype), torch.zeros(tokens, nq * d, dtype=dtype, device=DEVICE)
+    mass = torch.zeros(pool, nkv, page, device=DEVICE)
+    sms = ops._multiprocessors(torch.device(DEVICE))
+
+    def peak(call):
+        call()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        call()
+        return torch.cuda.max_memory_allocated() - before
+
+    attention = peak(lambda: ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, wide, nq, max(counts), longest, out=out, row_tokens=tuple(counts) if known else None))
+    masses = peak(lambda: ops.attention_mass(q, k_pages, mass, q_start, kv_len, wide, nq, max(counts), longest, last=votes))
+    plain_masses = peak(lambda: ops.attention_mass(q, torch.zeros_like(k_pages.codes).new_zeros((pool, nkv, page, d)).to(dtype), mass, q_start, kv_len, wide, nq, max(counts), longest, last=votes))
+    plain_masses -= pool * nkv * page * d * (1 + q.element_size())
+    for taken, packed, voting in ((attention, True, 0), (masses, False, votes), (plain_masses, False, votes)):
+        assert taken <= ops.compact_cache_workspace(rows, tokens, longest, nq, nkv, d, q.element_size(), packed, voting, sms), (packed, voting, taken)
+    ops.raise_on_kernel_errors(torch.device(DEVICE))

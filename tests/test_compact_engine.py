@@ -166,3 +166,42 @@ def test_a_model_refuses_for_its_mixers():
         model.compact_caches(CompactCache(4))
     model.compact_caches(CompactCache(keep=20))
     assert all(need.kv.keep == 20 for need in model.cache_needs())
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("bits, keep", [(16, None), (4, None), (4, 600), (16, 600)])
+def test_the_pool_leaves_room_for_workspaces(bits, keep, graphs, monkeypatch):
+    """Pages take what is left of the device's share after the weights, a step's activations and what a compact cache's operators take for a while."""
+    import torch
+
+    from pylon_b200.config import ARCHITECTURES, Qwen3Config
+    from pylon_b200.engine.engine import Engine
+    from pylon_b200.kernels import ops
+    from pylon_b200.models.decoder import DecoderModel
+
+    architecture = next(entry for entry in ARCHITECTURES.values() if entry.config_class is Qwen3Config)
+    fields = dict(TINY_CONFIGS["tinyC"], max_position_embeddings=40_960)
+    engine = Engine.__new__(Engine)
+    engine.device, engine.spec = None, architecture.build_spec(Qwen3Config(**fields), None)
+    engine.config = EngineConfig(dtype="bfloat16", page_size=64, max_batch_size=500, prefill_chunk_size=2048, max_gpu_utilization=1.0, cuda_graphs=graphs, cache_bits=bits, cache_keep=keep)
+    engine.model = DecoderModel(engine.spec)
+    compact = CompactCache(bits, keep=keep)
+    if bits == 4 or keep:
+        engine.model.compact_caches(compact)
+    for block in engine.model.blocks:
+        block.mixer.w_qkv = torch.zeros(1, dtype=torch.bfloat16)
+    monkeypatch.setattr(ops, "_multiprocessors", lambda device: 148)
+    total = 6 << 30
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (total - (1 << 30), total))
+    needs = engine.model.cache_needs()
+    pages = engine._pool_pages(needs, torch.bfloat16, 64)
+    held = sum(pages[need.kv] * 64 * need.kv.row_bytes(2) for need in needs)
+    heads, kv_heads, d = fields["num_attention_heads"], fields["num_key_value_heads"], fields["head_dim"]
+    longest = 40_960 if keep is None else min(40_960, keep + compact.slack + 2048 + 256 + 1000)
+    room = ops.compact_cache_workspace(1000, 2048 + 256 + 1000, longest, heads, kv_heads, d, 2, bits == 4, 64 if keep else 0, 148)
+    assert room > (1 << 29 if bits == 4 else 1 << 24 if keep else -1)
+    room = room * (2 if graphs else 1) if bits == 4 or keep else 0
+    left = total - (1 << 30) - 2048 * engine.spec.width * 64 - room
+    assert held <= left
+    if keep is None:   # (an evicting pool is no larger than what its requests may hold)
+        assert held > left - (1 << 20)
