@@ -115,7 +115,7 @@ class Engine:
         pool holds that many tokens; else it takes what is left of the allowed share of the device after the weights,
         less room for the activations of one full step and, with a compact cache, for its operators' workspace (raun6k/Pylon sizes its pool the same way,
         src/pylon/kv/budget.py:70-113).  A windowed group is given only what ``max_batch_size`` requests can hold of it
-        at once, and the groups that keep everything share the rest."""
+        at once, and the groups that keep everything share the rest; so do groups that evict, up to what their requests can hold."""
         slots, chunk, longest = self.config.max_batch_size, self.config.prefill_chunk_size, self.spec.max_positions
         if self.config.max_cache_tokens is not None:
             return group_page_counts(needs, page_size, self.config.max_cache_tokens, slots, longest, chunk)
@@ -133,13 +133,13 @@ class Engine:
             # (padded steps have up to twice the rows and an eighth more tokens; graphs keep a workspace of their own beside that of eager steps)
             activation_room += self.model.workspace_bytes(2 * slots, chunk + chunk // 8 + 2 * slots, longest) * (2 if self.config.cuda_graphs else 1)
         budget = int(total * self.config.max_gpu_utilization) - (total - free) - activation_room
-        windowed = {kv: pages for kv, pages in most.items() if kv.bounded}
+        windowed = {kv: pages for kv, pages in most.items() if kv.bounded and kv.keep is None}
         budget -= sum(pages * page_bytes[kv] for kv, pages in windowed.items())
-        shared = sum(size for kv, size in page_bytes.items() if not kv.bounded)
+        shared = sum(size for kv, size in page_bytes.items() if kv not in windowed)
         pages = budget // shared if shared else 0
         if budget < 0 or (shared and pages < 1):
             raise RuntimeError("no memory is left for the cache after loading the weights")
-        return {kv: (count if kv.bounded else int(min(pages, count))) for kv, count in most.items()}
+        return {kv: (count if kv in windowed else int(min(pages, count))) for kv, count in most.items()}
 
     # -- the step function, for callers that batch themselves --------------------------------
     def open(self, request_id: object, capacity: int) -> RequestCache:

@@ -168,10 +168,8 @@ def test_a_model_refuses_for_its_mixers():
     assert all(need.kv.keep == 20 for need in model.cache_needs())
 
 
-@pytest.mark.parametrize("graphs", [False, True])
-@pytest.mark.parametrize("bits, keep", [(16, None), (4, None), (4, 600), (16, 600)])
-def test_the_pool_leaves_room_for_workspaces(bits, keep, graphs, monkeypatch):
-    """Pages take what is left of the device's share after the weights, a step's activations and what a compact cache's operators take for a while."""
+def sized_engine(monkeypatch, total, **options):
+    """An engine without weights on a device of ``total`` bytes, 1 GB of them taken: what its pool is sized by."""
     import torch
 
     from pylon_b200.config import ARCHITECTURES, Qwen3Config
@@ -183,18 +181,27 @@ def test_the_pool_leaves_room_for_workspaces(bits, keep, graphs, monkeypatch):
     fields = dict(TINY_CONFIGS["tinyC"], max_position_embeddings=40_960)
     engine = Engine.__new__(Engine)
     engine.device, engine.spec = None, architecture.build_spec(Qwen3Config(**fields), None)
-    engine.config = EngineConfig(dtype="bfloat16", page_size=64, max_batch_size=500, prefill_chunk_size=2048, max_gpu_utilization=1.0, cuda_graphs=graphs, cache_bits=bits, cache_keep=keep)
+    engine.config = EngineConfig(dtype="bfloat16", page_size=64, max_batch_size=500, prefill_chunk_size=2048, max_gpu_utilization=1.0, **options)
     engine.model = DecoderModel(engine.spec)
-    compact = CompactCache(bits, keep=keep)
-    if bits == 4 or keep:
-        engine.model.compact_caches(compact)
+    if engine.config.cache_bits == 4 or engine.config.cache_keep:
+        engine.model.compact_caches(CompactCache(engine.config.cache_bits, keep=engine.config.cache_keep))
     for block in engine.model.blocks:
         block.mixer.w_qkv = torch.zeros(1, dtype=torch.bfloat16)
     monkeypatch.setattr(ops, "_multiprocessors", lambda device: 148)
-    total = 6 << 30
     monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (total - (1 << 30), total))
     needs = engine.model.cache_needs()
-    pages = engine._pool_pages(needs, torch.bfloat16, 64)
+    return engine, needs, engine._pool_pages(needs, torch.bfloat16, 64)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("bits, keep", [(16, None), (4, None), (4, 600), (16, 600)])
+def test_the_pool_leaves_room_for_workspaces(bits, keep, graphs, monkeypatch):
+    """Pages take what is left of the device's share after the weights, a step's activations and what a compact cache's operators take for a while."""
+    from pylon_b200.kernels import ops
+
+    total, fields = 6 << 30, TINY_CONFIGS["tinyC"]
+    engine, needs, pages = sized_engine(monkeypatch, total, cuda_graphs=graphs, cache_bits=bits, cache_keep=keep)
+    compact = CompactCache(bits, keep=keep)
     held = sum(pages[need.kv] * 64 * need.kv.row_bytes(2) for need in needs)
     heads, kv_heads, d = fields["num_attention_heads"], fields["num_key_value_heads"], fields["head_dim"]
     longest = 40_960 if keep is None else min(40_960, keep + compact.slack + 2048 + 256 + 1000)
@@ -205,3 +212,16 @@ def test_the_pool_leaves_room_for_workspaces(bits, keep, graphs, monkeypatch):
     assert held <= left
     if keep is None:   # (an evicting pool is no larger than what its requests may hold)
         assert held > left - (1 << 20)
+
+
+@pytest.mark.parametrize("keep", [600, 20_000, 40_000])
+def test_a_pool_that_evicts_takes_what_there_is(keep, monkeypatch):
+    """Requests that may keep more than the device has room for share what it has, as requests that keep everything do."""
+    from pylon_b200.cache.manager import group_page_counts
+
+    engine, needs, pages = sized_engine(monkeypatch, 6 << 30, cache_keep=keep)
+    most = group_page_counts(needs, 64, 500 * 40_960, 500, 40_960, 2048)
+    for need in needs:
+        assert 0 < pages[need.kv] <= most[need.kv]
+    held = sum(pages[need.kv] * 64 * need.kv.row_bytes(2) for need in needs)
+    assert held <= 5 << 30 and (keep == 600 or held > 3 << 30)
