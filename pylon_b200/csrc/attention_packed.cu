@@ -15,7 +15,9 @@
 //   Values, whose sums run over all keys, and keys whose weights are summed (float32 results) go through one half-precision multiply-add on another unit, which
 //     makes (code - zero) x 2^-10 of either, exactly and normal.
 //   A weight times the step of its values is one float16 number: the reference of the softmax is the running maximum of score + log2(step), not of the score,
-//     which keeps that product below 2^9 whatever the values' sizes.
+//     less LIFT, which keeps that product below 2^15 whatever the values' sizes.  Groups of channels whose steps differ are first brought to one size, by powers of two
+//     (up to 2^64) that follow the largest step of each group so far.  A product counts with float16's 11 bits down to 2^-20 of the largest, below that
+//     with an absolute error of 2^-31 of it at most: over n keys a channel is off by n x 2^-27 of its group's largest step at most, beside the rounding of weights.
 //
 // Layout.  Scores are computed transposed: 16 keys are the rows of an m16n8k16 product and the 8 or 16 packed query rows its columns, so no half of a tile
 // is empty with up to 8 query heads to a KV head.  Any order of the channels serves a product, so a thread takes 32 (64, 128) contiguous bits of a key's
@@ -49,6 +51,9 @@ constexpr int ROW_CHUNKS = D / 32;                        // 16-byte pieces of a
 constexpr int SMALL_ROWS = 16;
 constexpr float NOTHING = -3.0e38f;                       // a maximum before any score
 constexpr float RESCALE_STEP = 8.f;                       // log2: the reference maximum moves when a score is more than this above it
+constexpr float LIFT = 6.f;                               // log2: how far below the maximum the reference of weights that meet values is: 2^(6 + 8), times a mantissa, is float16's room
+constexpr float SMALLEST = -80.f;                         // log2 of a key's step, at least: a weight of 2^(80 + 14) leaves a sum room
+constexpr int MOST_APART = 64;                            // log2: groups are brought together by no more than this
 
 struct PackedParams {
   const __nv_bfloat16* q;
@@ -450,6 +455,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[gr][mt][nt][i] = 0.f;
     }
+    unsigned largest_steps = 0u, above = 0u;   // a byte to a group: exponent of its largest step so far; by how much that is above the least of the groups'
 
     for (int turn = 0; turn < tiles; ++turn) {
       copy_wait<STAGES - 1>();
@@ -468,6 +474,38 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
           for (int gr = 0; gr < GROUPS; ++gr) largest = max(largest, (unsigned)words[S::WORD_BYTES / 2 + gr]);
         }
         const bool bad = largest >= 0x7F80u;
+        if constexpr (!MASS && GROUPS > 1) {
+          unsigned steps = 0u;
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr) steps |= (bad ? 0u : (unsigned)words[S::WORD_BYTES / 2 + gr] >> 7) << (8 * gr);
+          if (__any_sync(0xffffffffu, __vcmpgtu4(steps, largest_steps) != 0u)) {   // rarely after the first tiles
+            int least = 255, most = 0;
+            unsigned next = 0u, next_above = 0u;
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+              const unsigned step = max((largest_steps >> (8 * gr)) & 255u, __reduce_max_sync(0xffffffffu, (steps >> (8 * gr)) & 255u));
+              next |= step << (8 * gr);
+              if (step) least = min(least, (int)step);
+              most = max(most, (int)step);
+            }
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+              const int step = (int)((next >> (8 * gr)) & 255u), old = (int)((above >> (8 * gr)) & 255u), now = max(0, min(MOST_APART, (step ? step : most) - least));   // (one of zeros: as the largest)
+              next_above |= (unsigned)now << (8 * gr);
+              if (now == old) continue;
+              const float factor = __uint_as_float((unsigned)(127 + old - now) << 23);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) o[gr][mt][nt][i] *= factor;
+            }
+            largest_steps = next;
+            above = next_above;
+          }
+        }
+        int size = 0;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr) {
           const unsigned word = words[gr];
@@ -475,11 +513,13 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
           key_scales[lane * GROUPS + gr] = make_float2(step, MASS ? __uint_as_float(as_bits(__float2half2_rn(zero * -0x1p-10f))) : step * zero);
           if constexpr (!MASS) {
             const unsigned value_word = words[S::WORD_BYTES / 2 + gr];
-            value_steps[lane * GROUPS + gr] = bad ? 0.f : word_step(value_word);
+            const int down = (int)((above >> (8 * gr)) & 255u);
+            value_steps[lane * GROUPS + gr] = bad ? 0.f : word_step(value_word) * __uint_as_float((unsigned)(127 - down) << 23);
+            size = max(size, (int)(value_word >> 7) - down);
             value_zeros[gr * WARP_KEYS + lane] = __float2half_rn(word_zero(value_word) * -0x1p-10f);
           }
         }
-        if constexpr (!MASS) value_sizes[lane] = largest < 16u || bad ? -100.f : (float)((int)(largest >> 7) - 127);
+        if constexpr (!MASS) value_sizes[lane] = bad ? SMALLEST : fmaxf(SMALLEST, (float)(size - 127));
       }
       __syncwarp();
 
@@ -577,7 +617,8 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
             }
       }
 
-      float most[NT][2];   // of score + log2 of the values' size
+      constexpr float lift = MASS ? 0.f : LIFT;
+      float most[NT][2];   // of score + log2 of the values' size, less the lift
       bool grows = false;
       float size[HALVES][2];
 #pragma unroll
@@ -591,8 +632,8 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
           float m = fmaxf(s[0][nt][i] + size[0][0], s[0][nt][2 + i] + size[0][1]);
 #pragma unroll
           for (int h = 1; h < HALVES; ++h) m = fmaxf(m, fmaxf(s[h][nt][i] + size[h][0], s[h][nt][2 + i] + size[h][1]));
-          most[nt][i] = m;
-          grows = grows || m > top[nt][i] + RESCALE_STEP;
+          most[nt][i] = m - lift;
+          grows = grows || most[nt][i] > top[nt][i] + RESCALE_STEP;
         }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -695,9 +736,10 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
 #pragma unroll
           for (int gr = 0; gr < GROUPS; ++gr) {
             float* to = merge_values + (size_t)(warp * COLUMNS + column) * D + gr * G + g * MINE;
+            const float back = __uint_as_float((137u + ((above >> (8 * gr)) & 255u)) << 23);   // 2^10, and the group's own size
 #pragma unroll
             for (int mt = 0; mt < MT; mt += 2)
-              *reinterpret_cast<float4*>(to + 2 * mt) = make_float4(1024.f * o[gr][mt][nt][i], 1024.f * o[gr][mt][nt][2 + i], 1024.f * o[gr][mt + 1][nt][i], 1024.f * o[gr][mt + 1][nt][2 + i]);
+              *reinterpret_cast<float4*>(to + 2 * mt) = make_float4(back * o[gr][mt][nt][i], back * o[gr][mt][nt][2 + i], back * o[gr][mt + 1][nt][i], back * o[gr][mt + 1][nt][2 + i]);
           }
         }
       }

@@ -229,3 +229,94 @@ def test_what_is_taken_for_a_while(dtype, nq, nkv, d, counts, longest, known):
     for taken, packed, voting in ((attention, True, 0), (masses, False, votes), (plain_masses, False, votes)):
         assert taken <= ops.compact_cache_workspace(rows, tokens, longest, nq, nkv, d, q.element_size(), packed, voting, sms), (packed, voting, taken)
     ops.raise_on_kernel_errors(torch.device(DEVICE))
+
+
+# ---------------------------------------------------------------------------------------
+# decoded tokens over the codes: values and scores of unlike sizes
+# ---------------------------------------------------------------------------------------
+def pages_of(rows, page, group):
+    """4-bit pages that hold ``rows [slots, nkv, d]`` one page after another, and their table."""
+    from pylon_b200.kernels import ops
+
+    slots, nkv, d = rows.shape
+    count = -(-slots // page)
+    full = torch.zeros(count * page, nkv, d, dtype=torch.float64, device=DEVICE)
+    full[:slots] = rows
+    return ops.PackedPages(*plain.pack(full.view(count, page, nkv, d).transpose(1, 2), group)), torch.arange(count, dtype=torch.int32, device=DEVICE)[None]
+
+
+def decoded(q, keys, values, group, page=64, scale=None):
+    """One bfloat16 token over ``keys`` and ``values [slots, nkv, d]``: the result, the result in 64 bits, the sum of the weights times the values' sizes, every channel's
+    rounding of weights (float16, times the step) and of scores (codes as subnormal numbers), as bounds."""
+    from pylon_b200.kernels import ops
+
+    slots, nkv, d = keys.shape
+    nq = q.shape[1] // d
+    scale = d ** -0.5 if scale is None else scale
+    k_pages, table = pages_of(keys, page, group)
+    v_pages, _ = pages_of(values, page, group)
+    got = ops.paged_attention_packed(q, k_pages, v_pages, ints([slots - 1]), ints([0]), ints([0, 1]), ints([slots]), table, nq, 1, slots, scale=scale)
+    ops.raise_on_kernel_errors(torch.device(DEVICE))
+    expected, size = plain.attention(q, k_pages, v_pages, [1], [slots], table, nq, scale)
+    largest = plain.steps(v_pages.words).amax((0, 2)).repeat_interleave(group, -1)                      # [nkv, d]: every group's largest step
+    terms = slots * 2.0 ** -27 * largest.repeat_interleave(nq // nkv, 0).flatten()
+    most = q.double().abs().view(nkv, nq // nkv, d).amax(1).unflatten(-1, (-1, group)).amax(-1)           # [nkv, groups]
+    score = scale * 15 * 2.0 ** -14 * float((plain.steps(k_pages.words).amax((0, 2)) * most).sum(-1).max())
+    share = 2.0 ** -11 + 2 * score + 4 * (d + 4) * 2.0 ** -24 * scale * float(torch.linalg.vector_norm(q.double().view(-1, d), dim=-1).max() * torch.linalg.vector_norm(keys, dim=-1).max())
+    return got.double(), expected, size, HALF[torch.bfloat16] * expected.abs() + share * size + terms
+
+
+@pytest.mark.parametrize("slots", [40, 700, 5000])
+@pytest.mark.parametrize("d, group", [(128, 32), (128, 64), (64, 32)])
+@pytest.mark.parametrize("apart", [0, 16, -16, 28, -28, 60])
+def test_groups_of_values_of_unlike_size(apart, d, group, slots):
+    """Every group is right by its own measure, however much larger the others are."""
+    nq, nkv = 8, 2
+    values = torch.randn(slots, nkv, d, dtype=torch.float64, device=DEVICE)
+    values[..., group:] *= 2.0 ** apart
+    q = torch.randn(1, nq * d, device=DEVICE).bfloat16()
+    got, expected, size, bound = decoded(q, torch.randn(slots, nkv, d, dtype=torch.float64, device=DEVICE), values, group)
+    assert ((got - expected).abs() <= bound).all(), float(((got - expected).abs() / size).max())
+
+
+@pytest.mark.parametrize("d, group", [(128, 32), (128, 64), (64, 32)])
+@pytest.mark.parametrize("apart", [20, -20, 40])
+@pytest.mark.parametrize("seen", [True, False])
+def test_a_late_key_whose_groups_are_of_unlike_size(seen, apart, d, group):
+    """A key far into the context whose first group alone is much larger (or all others are), seen or passed over: the other groups keep what they had."""
+    nq, nkv, slots = 8, 2, 3000
+    keys, values = (torch.randn(slots, nkv, d, dtype=torch.float64, device=DEVICE) for _ in range(2))
+    q = torch.randn(1, nq * d, device=DEVICE).bfloat16()
+    if not seen:      # its score is far below the others'
+        keys[2500] = -8 * q.double().view(nkv, nq // nkv, d).mean(1)
+    if apart > 0:
+        values[2500, :, :group] *= 2.0 ** apart
+    else:
+        values[2500, :, group:] *= 2.0 ** -apart
+    got, expected, size, bound = decoded(q, keys, values, group)
+    assert ((got - expected).abs() <= bound).all(), float(((got - expected).abs() / size).max())
+
+
+@pytest.mark.parametrize("d, group", [(128, 128), (128, 32), (64, 64)])
+@pytest.mark.parametrize("below, slots", [(10.0, 5_000), (16.6, 100_000), (18.0, 200_000)])
+def test_many_small_weights_beside_one(below, slots, d, group):
+    """One key far above a long flat context: the others' weights, e^-below each, still count where that key has no value."""
+    nq, nkv = 2, 1
+    keys, values = torch.zeros(slots, nkv, d, dtype=torch.float64, device=DEVICE), torch.ones(slots, nkv, d, dtype=torch.float64, device=DEVICE)
+    keys[slots // 3, :, 0] = below / 4
+    values[slots // 3] = 0.0
+    q = torch.zeros(1, nq * d, device=DEVICE).bfloat16()
+    q[:, ::d] = 4.0
+    got, expected, size, bound = decoded(q, keys, values, group, scale=1.0)
+    assert ((got - expected).abs() <= bound).all() and (bound <= 0.05 * expected).all(), (float(got.max()), float(expected.max()))
+
+
+@pytest.mark.parametrize("d, group", [(128, 128), (128, 64), (128, 32), (64, 64)])
+def test_scores_that_are_differences_of_large_sums(d, group):
+    """Queries of one sign over keys whose codes lie around the middle: the product over the codes is far larger than the score that is left of it.  A score is off by 2^-14 of
+    15 steps times the largest query, group by group."""
+    nq, nkv, slots = 8, 2, 300
+    keys = torch.randn(slots, nkv, d, dtype=torch.float64, device=DEVICE)
+    q = (3.0 + torch.rand(1, nq * d, device=DEVICE)).bfloat16()
+    got, expected, size, bound = decoded(q, keys * 0.05, torch.randn(slots, nkv, d, dtype=torch.float64, device=DEVICE), group, scale=1.0)
+    assert ((got - expected).abs() <= bound).all(), float(((got - expected).abs() / size).max())
