@@ -8,9 +8,10 @@
 // that make operands of codes, so the operands are chosen for few of them:
 //   A code in the lowest bits of a float16 is the subnormal number code x 2^-24, four bits further up code x 2^-20: masking alone makes operands, one shift and four
 //   masks for eight codes.
-//   Scores of an attention take them as they are (channels of odd number: the queries are divided by 16, which is exact).  A product of a subnormal number keeps
-//     some 14 bits below the largest one's code, 1e-4 of a score at most.  Queries are brought to [8, 16) by a power of two per packed row, so that every
-//     bfloat16 query has its place.  (Codes as e4m3 bytes would need three instructions, but this device makes float16 numbers of such operands again: 32.3
+//   Scores of an attention take them as they are (channels of odd number: the queries are divided by 16, which is exact).  A sum of products of subnormal numbers keeps
+//     some 14 bits below the largest query times the largest code, so a score is off by 2^-14 x 15 steps x the largest query in each group, times the scale.
+//     That is a bound on the sum over the codes, not on what is left of it: where step zero sum(q) cancels most of that (queries of one sign over keys around
+//     zero) it is no share of the score.  Queries are brought to [8, 16) by a power of two per packed row, so that every bfloat16 query has its place.  (Codes as e4m3 bytes would need three instructions, but this device makes float16 numbers of such operands again: 32.3
 //     against 27.8 million instructions over 16 x 8,192 keys.)
 //   Values, whose sums run over all keys, and keys whose weights are summed (float32 results) go through one half-precision multiply-add on another unit, which
 //     makes (code - zero) x 2^-10 of either, exactly and normal.

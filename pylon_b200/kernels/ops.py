@@ -2439,10 +2439,12 @@ def paged_attention_packed(
     Pages that a window has passed may be gone (-1 in the table).
 
     Head sizes: multiples of 32 up to 256.  bfloat16 queries of rows of at most 16 packed query rows (tokens x query heads of a KV head) run on a tensor-core kernel
-    over the codes where the head size is 64 or 128 (``csrc/attention_packed.cu``; scores and sums are 32-bit, a weight times the step of its values is rounded to
-    float16 once); longer rows on :func:`paged_attention`'s tensor-memory kernel (a tile's keys shared by several blocks where tiles are few) over
-    a workspace with their contexts unpacked, as do all bfloat16 rows of other head sizes; float32 queries run in 32 bits, few to a row on a kernel over
-    the codes, others on :func:`paged_attention` over unpacked contexts.  In bfloat16 a value that is not a number takes all channels of the heads that see it, not its group's alone."""
+    over the codes where the head size is 64 or 128 (``csrc/attention_packed.cu``).  A score is off there by at most ``scale * 2**-14 * 15 * step * max|q|``, summed over
+    the groups of a key; a weight times the step of its values is rounded to float16 once (11 bits, and 2^-31 of the largest); sums are 32-bit.  Longer rows run
+    on :func:`paged_attention`'s tensor-memory kernel (a tile's keys shared by several blocks where tiles are few) over a workspace with their contexts unpacked; so do
+    all bfloat16 rows of other head sizes, and single tokens with more than 16 query heads to a KV head, at the price of unpacking their whole contexts in every
+    call.  Weights there are rounded to bfloat16, 8 bits, before the weighted sum, as :func:`paged_attention` does without ``split_weights``.  float32 queries run in 32 bits, few to a row
+    on a kernel over the codes, others on :func:`paged_attention` over unpacked contexts.  In bfloat16 a value that is not a number takes all channels of the heads that see it, not its group's alone."""
     what = "paged_attention_packed"
     pages, nkv, page_size, d, group = _packed_pair(k_pages, v_pages, what)
     dtype_code = _dtype_code(q.dtype)
