@@ -456,7 +456,10 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[gr][mt][nt][i] = 0.f;
     }
-    unsigned largest_steps = 0u, above = 0u;   // a byte to a group: exponent of its largest step so far; by how much that is above the least of the groups'
+    // Of every group: the word from which on a step is larger than all so far; and, a byte each, the exponent of the power of two that brings its steps to the least group's.
+    unsigned larger_from[GROUPS], down = 0x7F7F7F7Fu;
+#pragma unroll
+    for (int gr = 0; gr < GROUPS; ++gr) larger_from[gr] = 128u;
 
     for (int turn = 0; turn < tiles; ++turn) {
       copy_wait<STAGES - 1>();
@@ -476,25 +479,25 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
         }
         const bool bad = largest >= 0x7F80u;
         if constexpr (!MASS && GROUPS > 1) {
-          unsigned steps = 0u;
+          bool larger = false;
 #pragma unroll
-          for (int gr = 0; gr < GROUPS; ++gr) steps |= (bad ? 0u : (unsigned)words[S::WORD_BYTES / 2 + gr] >> 7) << (8 * gr);
-          if (__any_sync(0xffffffffu, __vcmpgtu4(steps, largest_steps) != 0u)) {   // rarely after the first tiles
-            int least = 255, most = 0;
-            unsigned next = 0u, next_above = 0u;
+          for (int gr = 0; gr < GROUPS; ++gr) larger = larger || words[S::WORD_BYTES / 2 + gr] >= larger_from[gr];
+          if (__any_sync(0xffffffffu, larger && !bad)) {   // rarely after the first tiles
+            int step[GROUPS], least = 255, most = 0;
 #pragma unroll
             for (int gr = 0; gr < GROUPS; ++gr) {
-              const unsigned step = max((largest_steps >> (8 * gr)) & 255u, __reduce_max_sync(0xffffffffu, (steps >> (8 * gr)) & 255u));
-              next |= step << (8 * gr);
-              if (step) least = min(least, (int)step);
-              most = max(most, (int)step);
+              step[gr] = (int)max((larger_from[gr] >> 7) - 1u, __reduce_max_sync(0xffffffffu, bad ? 0u : (unsigned)words[S::WORD_BYTES / 2 + gr] >> 7));
+              larger_from[gr] = (unsigned)(step[gr] + 1) << 7;
+              if (step[gr]) least = min(least, step[gr]);
+              most = max(most, step[gr]);
             }
+            unsigned next = 0u;
 #pragma unroll
             for (int gr = 0; gr < GROUPS; ++gr) {
-              const int step = (int)((next >> (8 * gr)) & 255u), old = (int)((above >> (8 * gr)) & 255u), now = max(0, min(MOST_APART, (step ? step : most) - least));   // (one of zeros: as the largest)
-              next_above |= (unsigned)now << (8 * gr);
+              const int old = (int)((down >> (8 * gr)) & 255u), now = 127 - max(0, min(MOST_APART, (step[gr] ? step[gr] : most) - least));   // (one of zeros: as the largest)
+              next |= (unsigned)now << (8 * gr);
               if (now == old) continue;
-              const float factor = __uint_as_float((unsigned)(127 + old - now) << 23);
+              const float factor = __uint_as_float((unsigned)(127 + now - old) << 23);
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -502,8 +505,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
 #pragma unroll
                   for (int i = 0; i < 4; ++i) o[gr][mt][nt][i] *= factor;
             }
-            largest_steps = next;
-            above = next_above;
+            down = next;
           }
         }
         int size = 0;
@@ -514,13 +516,13 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
           key_scales[lane * GROUPS + gr] = make_float2(step, MASS ? __uint_as_float(as_bits(__float2half2_rn(zero * -0x1p-10f))) : step * zero);
           if constexpr (!MASS) {
             const unsigned value_word = words[S::WORD_BYTES / 2 + gr];
-            const int down = (int)((above >> (8 * gr)) & 255u);
-            value_steps[lane * GROUPS + gr] = bad ? 0.f : word_step(value_word) * __uint_as_float((unsigned)(127 - down) << 23);
-            size = max(size, (int)(value_word >> 7) - down);
+            const unsigned exponent = GROUPS > 1 ? (down >> (8 * gr)) & 255u : 127u;
+            value_steps[lane * GROUPS + gr] = bad ? 0.f : word_step(value_word) * __uint_as_float(exponent << 23);
+            size = max(size, (int)((value_word >> 7) + exponent));
             value_zeros[gr * WARP_KEYS + lane] = __float2half_rn(word_zero(value_word) * -0x1p-10f);
           }
         }
-        if constexpr (!MASS) value_sizes[lane] = bad ? SMALLEST : fmaxf(SMALLEST, (float)(size - 127));
+        if constexpr (!MASS) value_sizes[lane] = bad ? SMALLEST : fmaxf(SMALLEST, (float)(size - 254));
       }
       __syncwarp();
 
@@ -737,7 +739,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_an_sm(NT, MASS)) attention_
 #pragma unroll
           for (int gr = 0; gr < GROUPS; ++gr) {
             float* to = merge_values + (size_t)(warp * COLUMNS + column) * D + gr * G + g * MINE;
-            const float back = __uint_as_float((137u + ((above >> (8 * gr)) & 255u)) << 23);   // 2^10, and the group's own size
+            const float back = __uint_as_float((264u - (GROUPS > 1 ? (down >> (8 * gr)) & 255u : 127u)) << 23);   // 2^10, and the group's own size
 #pragma unroll
             for (int mt = 0; mt < MT; mt += 2)
               *reinterpret_cast<float4*>(to + 2 * mt) = make_float4(back * o[gr][mt][nt][i], back * o[gr][mt][nt][2 + i], back * o[gr][mt + 1][nt][i], back * o[gr][mt + 1][nt][2 + i]);
