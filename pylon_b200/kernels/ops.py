@@ -2478,7 +2478,7 @@ def paged_attention_packed(
     if tokens == 0 or rows == 0:
         return out
     if q.data_ptr() % 16 or q.stride(0) * q.element_size() % 16:   # the kernels read 16 bytes at once
-        q = q[:, : nq * d].contiguous()
+        q = q[:, : nq * d].clone(memory_format=torch.contiguous_format)   # (a single row counts as contiguous wherever it lies)
     group_heads, bf16 = nq // nkv, q.dtype == torch.bfloat16
     counts = tuple(row_tokens) if row_tokens is not None and len(row_tokens) == rows else None
     if max_q * group_heads > 16 or (bf16 and d not in (64, 128)):

@@ -320,3 +320,26 @@ def test_scores_that_are_differences_of_large_sums(d, group):
     q = (3.0 + torch.rand(1, nq * d, device=DEVICE)).bfloat16()
     got, expected, size, bound = decoded(q, keys * 0.05, torch.randn(slots, nkv, d, dtype=torch.float64, device=DEVICE), group, scale=1.0)
     assert ((got - expected).abs() <= bound).all(), float(((got - expected).abs() / size).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d, nq", [(128, 8), (64, 40), (96, 8)])
+def test_a_single_query_anywhere_in_memory(d, nq, dtype):
+    """One token's row counts as contiguous whatever its stride and its address."""
+    from pylon_b200.kernels import ops
+
+    nkv, page, counts, lengths = 2, 16, [1], [70]
+    table, pool, q_start, kv_len, row, slots = tables(counts, lengths, page)
+    k_pages, v_pages = random_pages(pool, nkv, page, d, 32), random_pages(pool, nkv, page, d, 32)
+    row_of = torch.randn(1, nq * d + 5, device=DEVICE).to(dtype)
+    results = []
+    for q in (row_of[:, :-5], row_of[:, 3:-2], row_of):
+        got = ops.paged_attention_packed(q, k_pages, v_pages, slots, row, q_start, kv_len, table, nq, 1, 70)
+        aligned = torch.empty(1, nq * d, dtype=dtype, device=DEVICE).copy_(q[:, : nq * d])
+        assert torch.equal(got, ops.paged_attention_packed(aligned, k_pages, v_pages, slots, row, q_start, kv_len, table, nq, 1, 70))
+        mass, other = torch.zeros(pool, nkv, page, device=DEVICE), torch.zeros(pool, nkv, page, device=DEVICE)
+        ops.attention_mass(q, k_pages, mass, q_start, kv_len, table, nq, 1, 70)
+        ops.attention_mass(aligned, k_pages, other, q_start, kv_len, table, nq, 1, 70)
+        torch.testing.assert_close(mass, other, rtol=1e-4, atol=1e-6)      # (scores in 32 bits, on another kernel where the row is off its alignment)
+        results.append(got)
+    ops.raise_on_kernel_errors(torch.device(DEVICE))
