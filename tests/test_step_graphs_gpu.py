@@ -54,3 +54,19 @@ def test_states_are_advanced_once(models):   # noqa: F811
         logits.append(portions(engine, list(tokens))[1])
         assert not graphs or engine.step_function.graphs.replays["padded"] >= 3
     torch.testing.assert_close(logits[0], logits[1], rtol=0, atol=1e-3 * float(logits[0].std()))
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+@pytest.mark.parametrize("bits, keep", [(4, None), (4, 48), (16, 48)])
+def test_prompts_in_many_portions_give_the_tokens_of_eager_steps(bits, keep, seed, tiny_folders):
+    """In float32, prompts of up to 200 tokens in portions of 32 beside decoded tokens of other requests: what is evicted, and so every token, is the same."""
+    from pylon_b200.sampling import SamplingParams
+
+    name, rng = "tinyC", np.random.default_rng(seed)
+    prompts = [rng.integers(0, TINY_CONFIGS[name]["vocab_size"], size=n).tolist() for n in rng.integers(1, 200, size=7)]
+    outcomes = []
+    for options in (dict(run_ahead=False), dict(cuda_graphs=True, run_ahead=False), dict(cuda_graphs=True)):
+        engine = engine_for(tiny_folders[name], name, "float32", cache_bits=bits, cache_keep=keep, prefill_chunk_size=32, max_batch_size=3, **options)
+        outcomes.append([result.output_ids for result in engine.generate(prompts, SamplingParams(max_new_tokens=30, temperature=0.0, ignore_eos=True))])
+        assert not options.get("cuda_graphs") or engine.step_function.graphs.replays["padded"] > 3
+    assert outcomes[0] == outcomes[1] == outcomes[2]
