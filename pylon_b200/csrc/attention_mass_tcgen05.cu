@@ -11,7 +11,7 @@
 // 25 warps: 16 of softmax (four warpgroups, each 64 scores of a row; two warpgroups with 128 took 45 us where these take 41), 8 that bring keys (copies of 16
 // bytes, or codes that become bfloat16 numbers on the way; four took 295 us over 131,072 packed keys where eight take 280) into a ring of three tiles in the 128-byte swizzle, one that
 // issues the products into two score buffers (2 x 256 columns: all of tensor memory; one block to an SM).
-// What bounds it: both passes need one exponential per score (16 a clock and SM, twice what the products take), and it runs at half that rate, by the latencies of
+// What its time goes by: both passes need one exponential per score (16 a clock and SM, twice what the products take), and run at half that rate (issue slots 54 and 45 %), by the latencies of
 // its loads of tensor memory and of its first tile (a pass over 500 keys takes 9 us).  64 voting tokens of 32 / 8 heads of 128: 41 us over 16,384 plain keys and 44 over
 // packed ones (96 and 94 for attention_mass_mma.cu's m16n8k16 products, whose rate bounds them), 262 and 280 over 131,072 (660 and 643).
 //

@@ -4,7 +4,7 @@
 // skipped here.
 //
 // Mathematics.  A key is k = step (code - zero) per group of channels, so a score is sum over the groups of step (q . code - zero sum(q)): the product
-// runs over the codes, and steps and zeros join per key and group, not per element.  What bounds the kernel is the logic instructions (64 lanes a cycle and SM)
+// runs over the codes, and steps and zeros join per key and group, not per element.  Most of the kernel's instructions are the logic ones (64 lanes a cycle and SM)
 // that make operands of codes, so the operands are chosen for few of them:
 //   A code in the lowest bits of a float16 is the subnormal number code x 2^-24, four bits further up code x 2^-20: masking alone makes operands, one shift and four
 //   masks for eight codes.
@@ -30,8 +30,9 @@
 // whole leave maximum, sum and weighted values in scratch memory and a second kernel joins them (a kernel of its own, not the last block to arrive: no
 // counters, nothing that two graphs could share).
 //
-// Measured: 64 rows of 8,192 slots, 32 / 8 heads of 128, groups of 128 channels 129 us (4.3 TB/s; issue slots 54 %, the logic unit 49 % busy), groups of 64 and 32 141 and
-// 171 (more steps and zeros to join); one row of 131,071 slots 45 us, of 600 slots 8.
+// Measured: 64 rows of 8,192 slots, 32 / 8 heads of 128, groups of 128 channels 131 us (4.2 TB/s), groups of 64 and 32 147 and 178 (more steps and zeros to join; bringing
+// groups of values to one size is 5 us of either); one row of 131,071 slots 46 us, of 600 slots 8.  What bounds it is latency: issue slots 54 %, the logic unit 49 %, DRAM 41 %
+// busy, the 11 or 12 warps an SM that its registers leave room for waiting most for fixed latencies.
 //
 // The same kernel without values keeps the scores instead (attention_mass: how much weight every key got), and the second kernel turns them into weights.
 #include "common.cuh"
@@ -208,8 +209,8 @@ __device__ __forceinline__ void cursor_next(Cursor& c, const PackedParams& p, co
   if (c.tile < total) cursor_set(c, p, starts, c.tile, warp);
 }
 
-// Blocks to an SM, as measured: more do not help what logic instructions bound and begin more runs.  64 rows of 8,192 slots, 32 / 8 heads, groups of 128 channels of
-// heads of 128: attention 129 us with three, 130 with four (126 registers), 137 with five; its scores alone 130, 112 and 120.  Heads of 64, groups of 64: 93, 91, 101 and
+// Blocks to an SM, as measured: more of them have fewer registers each and begin more runs.  64 rows of 8,192 slots, 32 / 8 heads, groups of 128 channels of
+// heads of 128: attention 131 us with three, 133 with four, 139 with five; its scores alone 130, 112 and 120.  Heads of 64, groups of 64: 93, 93, 102 and
 // 107, 94, 98.  16 packed rows, 16 rows of 3,000 slots, groups of 32 channels of 128: 43 with two, 46 with three; scores 34 and 32.
 constexpr int blocks_an_sm(int column_tiles, bool mass) {
   const int blocks = D == 64 || mass ? 4 : 3;

@@ -53,64 +53,64 @@ __global__ void __launch_bounds__(128) attention_packed_plain_kernel(const T* q,
   }
   // Without parts one stretch; else the parts z, z + gridDim.z, ... of those that the token sees.
   for (int segment = segments ? oldest / PLAIN_SEGMENT + blockIdx.z : 0; segment <= (segments ? min(newest / PLAIN_SEGMENT, segments - 1) : 0); segment += segments ? gridDim.z : 1) {
-  const int first = segments ? max(oldest, segment * PLAIN_SEGMENT) : oldest, last = segments ? min(newest, segment * PLAIN_SEGMENT + PLAIN_SEGMENT - 1) : newest;
+    const int first = segments ? max(oldest, segment * PLAIN_SEGMENT) : oldest, last = segments ? min(newest, segment * PLAIN_SEGMENT + PLAIN_SEGMENT - 1) : newest;
 #pragma unroll
-  for (int e = 0; e < WORDS * 8; ++e) sum[e] = 0.f;
-  float top = -INFINITY, total = 0.f;
-  // Every group of a warp makes the same number of turns, so that the shuffles have all lanes.
-  for (int base = first; base <= last; base += PLAIN_GROUPS) {
-    const int j = base + g;
-    int page = -1;
-    if (j <= last) {
-      page = block_table[(size_t)row * table_width + j / page_size];
-      if (page < 0 || page >= num_pages) {
-        if (s == 0 && error) atomicExch(error, PYLON_ERROR_BAD_PAGE);
-        page = -1;
+    for (int e = 0; e < WORDS * 8; ++e) sum[e] = 0.f;
+    float top = -INFINITY, total = 0.f;
+    // Every group of a warp makes the same number of turns, so that the shuffles have all lanes.
+    for (int base = first; base <= last; base += PLAIN_GROUPS) {
+      const int j = base + g;
+      int page = -1;
+      if (j <= last) {
+        page = block_table[(size_t)row * table_width + j / page_size];
+        if (page < 0 || page >= num_pages) {
+          if (s == 0 && error) atomicExch(error, PYLON_ERROR_BAD_PAGE);
+          page = -1;
+        }
       }
+      const size_t at = ((size_t)max(page, 0) * nkv + kv_head) * page_size + (page >= 0 ? j % page_size : 0);
+      float x[WORDS * 8], score = 0.f;
+      plain_values<WORDS>(k_pages, k_words, at, s, d, group, x);
+#pragma unroll
+      for (int e = 0; e < WORDS * 8; ++e) score = fmaf(mine[e], x[e], score);
+#pragma unroll
+      for (int offset = 4; offset > 0; offset >>= 1) score += __shfl_xor_sync(0xffffffffu, score, offset);
+      if (page < 0) continue;
+      const float now = fmaxf(top, score);
+      if (now == -INFINITY && score == score) continue;   // nothing has weight yet
+      const float keep = expf(top - now), weight = expf(score - now);
+      plain_values<WORDS>(v_pages, v_words, at, s, d, group, x);
+      total = total * keep + weight;
+#pragma unroll
+      for (int e = 0; e < WORDS * 8; ++e) sum[e] = sum[e] * keep + weight * x[e];
+      top = now;
     }
-    const size_t at = ((size_t)max(page, 0) * nkv + kv_head) * page_size + (page >= 0 ? j % page_size : 0);
-    float x[WORDS * 8], score = 0.f;
-    plain_values<WORDS>(k_pages, k_words, at, s, d, group, x);
 #pragma unroll
-    for (int e = 0; e < WORDS * 8; ++e) score = fmaf(mine[e], x[e], score);
+    for (int e = 0; e < WORDS * 8; ++e) shared_out[g][64 * (e >> 3) + 8 * s + (e & 7)] = sum[e];
+    if (s == 0) {
+      shared_top[g] = top;
+      shared_total[g] = total;
+    }
+    __syncthreads();
+    float all = -INFINITY, denominator = 0.f;
 #pragma unroll
-    for (int offset = 4; offset > 0; offset >>= 1) score += __shfl_xor_sync(0xffffffffu, score, offset);
-    if (page < 0) continue;
-    const float now = fmaxf(top, score);
-    if (now == -INFINITY && score == score) continue;   // nothing has weight yet
-    const float keep = expf(top - now), weight = expf(score - now);
-    plain_values<WORDS>(v_pages, v_words, at, s, d, group, x);
-    total = total * keep + weight;
+    for (int i = 0; i < PLAIN_GROUPS; ++i) all = fmaxf(all, shared_top[i]);
+    float factor[PLAIN_GROUPS];
 #pragma unroll
-    for (int e = 0; e < WORDS * 8; ++e) sum[e] = sum[e] * keep + weight * x[e];
-    top = now;
-  }
+    for (int i = 0; i < PLAIN_GROUPS; ++i) {
+      factor[i] = shared_total[i] == 0.f ? 0.f : expf(shared_top[i] - all);
+      denominator += shared_total[i] * factor[i];
+    }
+    const size_t part = ((size_t)token * nq + head) * segments + segment;
+    if (segments && threadIdx.x == 0) part_sums[part] = make_float2(all, denominator);
+    for (int c = threadIdx.x; c < d; c += 128) {
+      float value = 0.f;
 #pragma unroll
-  for (int e = 0; e < WORDS * 8; ++e) shared_out[g][64 * (e >> 3) + 8 * s + (e & 7)] = sum[e];
-  if (s == 0) {
-    shared_top[g] = top;
-    shared_total[g] = total;
-  }
-  __syncthreads();
-  float all = -INFINITY, denominator = 0.f;
-#pragma unroll
-  for (int i = 0; i < PLAIN_GROUPS; ++i) all = fmaxf(all, shared_top[i]);
-  float factor[PLAIN_GROUPS];
-#pragma unroll
-  for (int i = 0; i < PLAIN_GROUPS; ++i) {
-    factor[i] = shared_total[i] == 0.f ? 0.f : expf(shared_top[i] - all);
-    denominator += shared_total[i] * factor[i];
-  }
-  const size_t part = ((size_t)token * nq + head) * segments + segment;
-  if (segments && threadIdx.x == 0) part_sums[part] = make_float2(all, denominator);
-  for (int c = threadIdx.x; c < d; c += 128) {
-    float value = 0.f;
-#pragma unroll
-    for (int i = 0; i < PLAIN_GROUPS; ++i) value += shared_out[i][c] * factor[i];
-    if (segments) part_values[part * d + c] = value;
-    else out[(size_t)token * out_stride + (size_t)head * d + c] = from_float<T>(denominator == 0.f ? 0.f : value / denominator);
-  }
-  __syncthreads();   // the groups' sums are free again
+      for (int i = 0; i < PLAIN_GROUPS; ++i) value += shared_out[i][c] * factor[i];
+      if (segments) part_values[part * d + c] = value;
+      else out[(size_t)token * out_stride + (size_t)head * d + c] = from_float<T>(denominator == 0.f ? 0.f : value / denominator);
+    }
+    __syncthreads();   // the groups' sums are free again
   }
 }
 

@@ -58,7 +58,8 @@ class CompactCache:
 
     ``bits``: 16, rows in the compute dtype; 4, rows in 4 bits (:class:`~pylon_b200.kernels.ops.PackedPages`), a scale for every ``group`` channels.
     ``keep``: a request's tokens beyond this many are evicted, each KV head choosing for itself: kept are the first ``keep_first`` tokens, the ``keep_recent``
-    newest and, of the others, those that the attention weighed most (of a step's tokens the last ``votes`` of each request vote).  Eviction waits for
+    newest and, of the others, those that the attention weighed most (of a step's tokens the last ``votes`` of each request vote, so that a prompt cut into more
+    portions has more voters, and its early portions lose tokens before the later ones vote).  Eviction waits for
     ``slack`` more tokens, so that it need not run at every step.  ``None``: nothing is evicted."""
 
     bits: int = 16
