@@ -124,6 +124,7 @@ class StepGraphs:
         function = self.step_function
         collector_was_on = gc.isenabled()
         gc.disable()   # destroying an old graph or a pinned buffer in mid-capture would invalidate it
+        saved_state = None
         try:
             # One eager run first: libraries are built and loaded, kernels configured, the
             # allocator warmed.  It writes the same cache slots the replay writes again; a state
@@ -143,6 +144,7 @@ class StepGraphs:
             # raun6k/Pylon logs "cuda_graph_capture_failed" and goes on eagerly
             # (src/pylon/decode/warmup.py:123-137); so does this engine.
             self.failed.add(key)
+            self.cache.restore_state(saved_state)   # (a first run that failed half way has advanced some layers)
             print(f"[pylon_b200] cuda graph capture failed for step size {key}: {error!r}", file=sys.stderr, flush=True)
             torch.cuda.synchronize(self.device)
             return None

@@ -53,3 +53,21 @@ def test_a_portion_that_is_replayed_does_not_run_again(want, monkeypatch):
     graphs.captured_padded, graphs.seen_padded, graphs.capture_at_once = {}, {}, False
     function([StepEntry(Request(), list(range(32)), want)])
     assert len(eager) == 1 and replayed == ["padded"]
+
+
+def test_a_capture_that_fails_half_way_puts_states_back(monkeypatch):
+    """The step runs eagerly after that: what the failed run had advanced already must not be advanced again."""
+    cache = Cache()
+    cache.save_state = lambda requests: cache.log.append("save") or ["saved"]
+    cache.restore_state = lambda saved: cache.log.append(("restore", saved))
+
+    def forward(step, caches):
+        cache.log.append("forward")
+        raise RuntimeError("no memory")
+
+    graphs = StepGraphs.__new__(StepGraphs)
+    graphs.cache, graphs.failed, graphs.device, graphs.pool = cache, set(), None, None
+    graphs.step_function = SimpleNamespace(model=SimpleNamespace(forward=forward))
+    monkeypatch.setattr(graphs_module, "torch", SimpleNamespace(cuda=SimpleNamespace(synchronize=lambda device: None)))
+    assert graphs._capture("key", None, [], None, None, []) is None
+    assert cache.log == ["save", "forward", ("restore", ["saved"])] and graphs.failed == {"key"}
